@@ -317,8 +317,6 @@ def _words(words):
 def prepare(case, seed):
     v = _inputs(case, seed)
     state = {"case": case, **(_library_state(case, v) if own else _plain_state(case, v))}
-    if own:
-        state["views"] = {k: _view(state[k]) for k in ("out", "kt", "vc") if k in state}
     torch.cuda.synchronize()
     return state
 
@@ -388,14 +386,14 @@ def run(state):
     if path == "q8_cache":
         ex.q8_cache_write(s["k"], s["v"], s["cache"], s["write"])
         ex.q8_cache_read(s["cache"], s["kt"], s["vc"], s["read"])
-        return {"kt": s["views"]["kt"], "v": s["views"]["vc"]}
+        return {"kt": _view(s["kt"]), "v": _view(s["vc"])}
     if path == "rope_axes":
         ex.rope_axes(s["x"], s["table"], s["pos"], s["out"], s["desc"])
     elif "cache" in s:
         ex.q8_tree_attention(s["q"], s["cache"], s["out"], s["desc"], mask=s["mask"])
     else:
         ex.tree_attention(s["q"], s["kt"], s["v"], s["out"], s["desc"], mask=s["mask"])
-    return s["views"]["out"]
+    return _view(s["out"])
 
 
 # --------------------------------------------------------------------- work
