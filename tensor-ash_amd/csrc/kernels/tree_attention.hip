@@ -30,12 +30,14 @@
 //  * f16 caches go through LDS tiles that the row tiles share, loaded directly
 //    and read transposed, while q's operands stay in registers.
 //
-// Precision (f32 activations: all within f32's own rounding):
+// Precision (f32 activations: all within a few of f32's own roundings, but
+// for the floor of small weights over f16 caches):
 //  * f32 caches: v_mfma_f32_32x32x2_f32, whole values;
 //  * f16 caches: f16 matrix cores.  f32 q, scaled by a power of two per row,
 //    in three f16 pieces, weights in two, the pieces after the first scaled up
-//    and summed apart; f16 q as it is, weights in two pieces, or one on the
-//    larger workgroups (TreeF16::NP);
+//    and summed apart: a weight within 2^-22 of itself, and within 2^-47 of its
+//    row's largest where it is below 2^-25 of that.  f16 q as it is, weights in
+//    two pieces: within 2^-22, or 2^-36 of the row's largest;
 //  * 8-bit cache: codes are exact in bf16, and so are f32 q and weights in
 //    three bf16 pieces of 8 bits.  f16 q meets the codes as f16, with weights
 //    in two bf16 pieces (2^-16 of a weight, below the result's own 2^-11).
@@ -925,13 +927,6 @@ template <int DH, bool IO16, bool DIRECT, int QB, int KP, int BKW> struct TreeF1
   static constexpr int KS = DH / 16, DB = DH / 32;
   static constexpr int NQ = IO16 ? 1 : 3;    // f16 pieces of q
   static constexpr int AHEAD = IO16 ? 4 : 2; // LDS reads before their use
-  // f16 pieces of the weights.  One, off by half a step of each weight (2^-11
-  // of it, as much as the rounding of an f16 result), where f16 activations
-  // bring more rows than 64: there the matrix cores bound the kernel, and the
-  // second piece's products took 11 of 61 us (64 tokens, 32704 positions, 32 / 8
-  // heads, dh 128).  Both go into one sum for f16 activations; for f32 ones
-  // the second is scaled up and summed apart.
-  static constexpr int NP = IO16 && QB == 4 ? 1 : 2;
   static constexpr int K_BYTES = DH * BK * 2, STAGE = 2 * K_BYTES;
   static constexpr int CK = BK / 8, CV = DH / 8; // 16-byte pieces per K / V row
   static constexpr int LD = K_BYTES / 16 / T;    // direct loads per thread, per operand
@@ -1138,6 +1133,12 @@ template <int DH, bool IO16, bool DIRECT, int QB, int KP, int BKW> struct TreeF1
     // 16u + 4h + 0..3 and 16u + 8 + 4h + 0..3) with the same V rows.
     // Operands are read `AHEAD` steps before their use: one by one, every
     // step waited for the LDS.
+    // A weight x (2^11 .. 2^15 where it is its row's largest) goes in two f16
+    // pieces, hi and the rest of it: within 2^-22 of itself, and below 2^-14 of
+    // the row's largest within 2^-36 of that (half of f16's smallest step).  For
+    // f16 activations both go into one sum; for f32 ones the second is scaled up
+    // and summed apart, which takes the floor to 2^-47.  hi alone would be off by
+    // 2^-11 of each weight, all of them to one side where weights coincide.
     f16x8 hi[KB][2], lo[KB][2];
     auto product = [&](uint32_t from) __attribute__((always_inline)) {
       const uint32_t at0 = lds0 + from * STAGE;
@@ -1160,9 +1161,9 @@ template <int DH, bool IO16, bool DIRECT, int QB, int KP, int BKW> struct TreeF1
         if (i % (KB * 2) == 0)
           rest = f32x16{};
         st.o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i], hi[kb][u], st.o[b], 0, 0, 0);
-        if constexpr (IO16 && NP > 1)
+        if constexpr (IO16)
           st.o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i], lo[kb][u], st.o[b], 0, 0, 0);
-        else if constexpr (NP > 1)
+        else
           rest = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i], lo[kb][u], rest, 0, 0, 0);
         in_order();
         if constexpr (!IO16) {
@@ -1266,8 +1267,7 @@ template <int DH, bool IO16, bool DIRECT, int QB, int KP, int BKW> struct TreeF1
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               hi[kb][u][e + i] = a[i];
-              if constexpr (NP > 1)
-                lo[kb][u][e + i] = IO16 ? (_Float16)(x[i] - (float)a[i])
+              lo[kb][u][e + i] = IO16 ? (_Float16)(x[i] - (float)a[i])
                                       : (_Float16)fmaf((float)a[i], -kLowScale, x[i] * kLowScale);
             }
           }

@@ -653,6 +653,43 @@ def test_tree_attention_without_scratch(ta, ctx, monkeypatch):
     c.check(c.run())
 
 
+# The sizes pick every kernel over f16 caches: 32, 64 (dh 128) and 128 rows to
+# a workgroup, rows of K in whole 16-byte pieces or not; the last two take the
+# 128-row kernel for the cache's capacity, the length being named by a cell.
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("group,tokens,t_max,cell", [
+    (1, 1, 256, False), (1, 1, 257, False), (8, 8, 256, False), (8, 8, 257, False), (64, 64, 256, False),
+    (64, 64, 257, False), (4, 64, 4104, True), (4, 64, 4103, True)])
+def test_tree_attention_f16_weights_in_two_pieces(ta, ex, dh, group, tokens, t_max, cell):
+    """f16 activations over an f16 cache hold weights in two f16 pieces, in a
+    prepared step as in an eager call: within 2^-22, counted twice (its own,
+    and the total's).  Half of the keys have the row's largest weight, which
+    f16 holds, the others one that it misses by nearly half a step, and V makes
+    their sums cancel, so that the result's own step is far below that."""
+    n = 256
+    c = Case(ta, ex, "f16", True, dh, 1, group, tokens, n - tokens, t_max - n, words=[(1 << tokens) - 1] * tokens)
+    d = np.arange(1, 512) / 64.0
+    w = np.exp(-4.0 * d * c.scale)
+    off = np.abs((w * 2048).astype(np.float16).astype(np.float64) / (w * 2048) - 1) * (w > 0.25) * (w < 0.9)
+    at = int(off.argmax())
+    assert off[at] > 0.75 * 2.0 ** -11
+    c.q[:] = 0.0
+    c.q.reshape(tokens, -1, dh)[..., 0] = 4.0
+    c.k[:] = 0.0
+    c.k[1::2, :, 0] = -d[at]
+    c.v[0::2] = 1.0
+    c.v[1::2] = np.float32(np.float16(-1.0 / w[at]))
+    c.put()
+    pos = ex.create_pos_buffer()
+    pos.set(n - tokens)
+    got = c.run(desc=c.desc(kv_len=0, pos_addr=pos.device_address) if cell else None)
+    out, mag, eps = c.ref()
+    tol = mag * (2 * (eps + 4 * U32) + 2 * n * U32 + 2.0 ** -21) + 2.0 ** -11 * np.abs(out) + 2.0 ** -25
+    # one piece would be off by that step of half of mag
+    assert (2 * tol < mag * off[at] / 2).all()
+    assert (np.abs(got - out) <= tol).all(), float((np.abs(got - out) / tol).max())
+
+
 # ------------------------------------------------------------- used together
 
 
