@@ -470,29 +470,6 @@ template <int DH, bool IO16, bool DIRECT, int QB, int KP, int BKW> struct FlashH
   static_assert(LD * T * 16 == K_BYTES && CK >= 8 && CV >= 8, "stages split evenly");
   static_assert(SMEM <= 160 * 1024, "LDS");
 
-  typedef short s16x4 __attribute__((ext_vector_type(4)));
-  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-
-  static TA_DEVICE uint32_t swz(uint32_t row, int chunks) {
-    return chunks >= 16 ? (0xACA60u >> (4u * (row & 3u))) & 15u : 2u * (row & 3u);
-  }
-  // `base` and `lds` are the same in every lane.
-  static TA_DEVICE void load16s(const void *src, uint32_t off, uint32_t lds) {
-    const uint64_t a = reinterpret_cast<uint64_t>(src);
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a);
-    const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
-    const uint64_t base = (uint64_t)lo | (uint64_t)hi << 32;
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds)
-                 : "memory", "m0");
-  }
-  // Two transpose reads: rows r .. r + 3 (`lo`) and r' .. r' + 3 (`hi`) of
-  // this lane's column.
-  static TA_DEVICE f16x8 tr(uint32_t lo, uint32_t hi) {
-    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(uintptr_t)lo);
-    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(uintptr_t)hi);
-    return __builtin_bit_cast(f16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
-  }
-
   static TA_DEVICE void run(const FlashArgs &p) {
     __shared__ __attribute__((aligned(1024))) char smem[SMEM];
     const uint32_t tid = threadIdx.x, lane = tid & 63u;
@@ -596,9 +573,9 @@ template <int DH, bool IO16, bool DIRECT, int QB, int KP, int BKW> struct FlashH
 #pragma unroll
     for (int i = 0; i < LD; ++i) {
       const uint32_t q = i * T + tid;
-      uint32_t row = q / CK, c = (q % CK) ^ swz(row, CK);
+      uint32_t row = q / CK, c = (q % CK) ^ ta_swizzle16(row, CK);
       koff[i] = row * p.t_max + 8u * c;
-      row = q / CV, c = (q % CV) ^ swz(row, CV);
+      row = q / CV, c = (q % CV) ^ ta_swizzle16(row, CV);
       voff[i] = row * DH + 8u * c;
     }
     // K rows that are not whole 16-byte pieces go through registers:
@@ -614,19 +591,19 @@ template <int DH, bool IO16, bool DIRECT, int QB, int KP, int BKW> struct FlashH
         if (whole) {
 #pragma unroll
           for (int i = 0; i < LD; ++i)
-            load16s(ks, koff[i] * 2u, base + i * T * 16u);
+            ta_load_lds16_uniform(ks, koff[i] * 2u, base + i * T * 16u);
         } else {
 #pragma unroll
           for (int i = 0; i < LD; ++i) {
             const uint32_t row = (i * T + tid) / CK, key = k0 + koff[i] - row * p.t_max;
-            load16s(kt, (row * p.t_max + min(key, p.t_max - 8u)) * 2u, base + i * T * 16u);
+            ta_load_lds16_uniform(kt, (row * p.t_max + min(key, p.t_max - 8u)) * 2u, base + i * T * 16u);
           }
         }
       } else {
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
           typedef f16x8 f16x8u __attribute__((aligned(2)));
-          const uint32_t q = i * T + tid, row = q / CK, c = (q % CK) ^ swz(row, CK);
+          const uint32_t q = i * T + tid, row = q / CK, c = (q % CK) ^ ta_swizzle16(row, CK);
           const uint64_t at = (uint64_t)row * p.t_max + k0 + 8u * c;
           if (at + 8u <= k_left) {
             kreg[i] = *reinterpret_cast<const f16x8u *>(kt + at);
@@ -640,12 +617,12 @@ template <int DH, bool IO16, bool DIRECT, int QB, int KP, int BKW> struct FlashH
       if (whole) {
 #pragma unroll
         for (int i = 0; i < LD; ++i)
-          load16s(vs, voff[i] * 2u, base + K_BYTES + i * T * 16u);
+          ta_load_lds16_uniform(vs, voff[i] * 2u, base + K_BYTES + i * T * 16u);
       } else {
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
           const uint32_t row = (i * T + tid) / CV;
-          load16s(vs, (voff[i] + (min(k0 + row, p.t_max - 1u) - k0 - row) * DH) * 2u,
+          ta_load_lds16_uniform(vs, (voff[i] + (min(k0 + row, p.t_max - 1u) - k0 - row) * DH) * 2u,
                   base + K_BYTES + i * T * 16u);
         }
       }
@@ -666,13 +643,13 @@ template <int DH, bool IO16, bool DIRECT, int QB, int KP, int BKW> struct FlashH
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
         const uint32_t col = kh * BKW + kb * 32u + 16u * (g & 1u) + 4u * (t16 & 3u);
-        k_off[kb] = row * (BK * 2) + 16u * ((col >> 3) ^ swz(row, CK)) + (col & 7u) * 2u;
+        k_off[kb] = row * (BK * 2) + 16u * ((col >> 3) ^ ta_swizzle16(row, CK)) + (col & 7u) * 2u;
       }
       const uint32_t vrow = kh * BKW + 4u * (g >> 1) + (t16 >> 2);
 #pragma unroll
       for (int b = 0; b < DB; ++b) {
         const uint32_t col = b * 32u + 16u * (g & 1u) + 4u * (t16 & 3u);
-        v_off[b] = K_BYTES + vrow * (DH * 2) + 16u * ((col >> 3) ^ swz(vrow, CV)) + (col & 7u) * 2u;
+        v_off[b] = K_BYTES + vrow * (DH * 2) + 16u * ((col >> 3) ^ ta_swizzle16(vrow, CV)) + (col & 7u) * 2u;
       }
     }
 
@@ -712,7 +689,7 @@ template <int DH, bool IO16, bool DIRECT, int QB, int KP, int BKW> struct FlashH
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
           const uint32_t at = st + k_off[kb] + ks * 16 * (BK * 2);
-          const f16x8 a = tr(at, at + 4 * (BK * 2));
+          const f16x8 a = ta_read_tr16(at, at + 4 * (BK * 2));
 #pragma unroll
           for (int q = 0; q < QP; ++q) {
             f32x16 &c = q ? low[kb] : s[kb];
@@ -793,7 +770,7 @@ template <int DH, bool IO16, bool DIRECT, int QB, int KP, int BKW> struct FlashH
           }
       auto v_at = [&](int b, int kb, int u) __attribute__((always_inline)) {
         const uint32_t at = st + v_off[b] + (kb * 32 + u * 16) * (DH * 2);
-        return tr(at, at + 8 * (DH * 2));
+        return ta_read_tr16(at, at + 8 * (DH * 2));
       };
       if constexpr (APART) {
 #pragma unroll

@@ -20,6 +20,51 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 // per SIMD.  y >= 1 wherever it is used here; rcp(inf) = 0.
 TA_DEVICE float ta_fast_div(float x, float y) { return x * __builtin_amdgcn_rcpf(y); }
 
+// ---- Direct global -> LDS loads: 16 bytes a lane, to lds + 16 * lane.  The
+// compiler's own wait states do not reach into inline code, so these hold
+// them: one between the write of m0 and the load, and five between a vector
+// instruction that writes a scalar register and a load that has it as its
+// base.  `lds`, and `base`, are the same in every lane.
+
+// From each lane's own address.
+TA_DEVICE void ta_load_lds16(const void *src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds)
+               : "memory", "m0");
+}
+// From base + off; `base` comes of scalar instructions alone.
+TA_DEVICE void ta_load_lds16(const void *base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds)
+               : "memory", "m0");
+}
+// The same pointer in every lane, moved to scalar registers.
+template <class T> TA_DEVICE const T *ta_uniform(const T *p) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a); // (the builtin's result is signed)
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
+  return reinterpret_cast<const T *>((uint64_t)lo | (uint64_t)hi << 32);
+}
+// From base + off, `base` the same in every lane wherever it was computed.
+TA_DEVICE void ta_load_lds16_uniform(const void *base, uint32_t off, uint32_t lds) {
+  const char *b = ta_uniform(static_cast<const char *>(base));
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(b), "s"(lds)
+               : "memory", "m0");
+}
+
+// Rows of `chunks` 16-byte pieces in LDS: piece c of row r lies at c ^ this,
+// which keeps the transpose reads of four rows apart.
+TA_DEVICE uint32_t ta_swizzle16(uint32_t row, int chunks) {
+  return chunks >= 16 ? (0xACA60u >> (4u * (row & 3u))) & 15u : 2u * (row & 3u);
+}
+// Two transpose reads of LDS: rows r .. r + 3 (`lo`) and r' .. r' + 3 (`hi`) of
+// this lane's column.
+TA_DEVICE f16x8 ta_read_tr16(uint32_t lo, uint32_t hi) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(uintptr_t)lo);
+  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(uintptr_t)hi);
+  return __builtin_bit_cast(f16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
 // Activation of the fused epilogue (shaders/matmul_epilogue_common.glsl:
 // 30-39 semantics), one instantiation per activation so an epilogue loop
 // specialised on it has no per-element branches.  exp is HIP's fast

@@ -290,11 +290,6 @@ struct GemmH16Pipe {
     return CPR >= 16 ? (0xACA60u >> (4u * (row & 3u))) & 15u : 2u * (row & 3u);
   }
 
-  static TA_DEVICE void load16(const void *src, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds)
-                 : "memory", "m0");
-  }
-
   struct Frags {
     f16x8 a[KS][FM], b[WAYS][KS][FN];
   };
@@ -381,14 +376,14 @@ struct GemmH16Pipe {
       const uint32_t base = lds0 + stage * STAGE + wave * 64 * 16;
 #pragma unroll
       for (int i = 0; i < A_LD; ++i) {
-        load16(asrc[i], base + i * T * 16);
+        ta_load_lds16(asrc[i], base + i * T * 16);
         asrc[i] += BK * 2;
       }
 #pragma unroll
       for (int w = 0; w < WAYS; ++w)
 #pragma unroll
         for (int i = 0; i < B_LD; ++i) {
-          load16(bsrc[w][i], base + A_BYTES + w * B_BYTES + i * T * 16);
+          ta_load_lds16(bsrc[w][i], base + A_BYTES + w * B_BYTES + i * T * 16);
           bsrc[w][i] += b_step;
         }
     };

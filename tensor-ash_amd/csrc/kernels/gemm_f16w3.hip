@@ -87,9 +87,7 @@ template <int FM, int NS, bool ALIGNED> struct GemmW3 {
         if (i * W + W > A_KB && wave >= (uint32_t)A_MORE)
           continue;
         const uint32_t l = lds0 + st * STAGE + (i * W + wave) * 1024u;
-        const char *a = asrc[i];
-        asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lo), "s"(a), "s"(l)
-                     : "memory", "m0");
+        ta_load_lds16(asrc[i], lo, l);
         asrc[i] += KS * STEP;
       }
 #pragma unroll
@@ -101,8 +99,7 @@ template <int FM, int NS, bool ALIGNED> struct GemmW3 {
           const char *src =
               reinterpret_cast<const char *>(B + k * p.n + min(n0 + 8u * c, p.n - 8u));
           const uint32_t l = lds0 + st * STAGE + A_KB * 1024u + (i * T + wave * 64u) * 16u;
-          asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(l)
-                       : "memory", "m0");
+          ta_load_lds16(src, l);
         } else {
           typedef f16x8 f16x8u __attribute__((aligned(2)));
           const uint64_t at = k * p.n + n0 + 8u * c; // columns past N reach into the next row

@@ -205,15 +205,9 @@ template <int BM, int BN, int WGM, int WGN, int NS> struct GemmF32Mi16 {
       const uint32_t jj = min(j, kts - 1u);
       const uint32_t base = lds0 + (j % NS) * STAGE + wave * 64 * 16;
       if constexpr (i < A_LD) {
-        const char *sb = abase0 + (uint64_t)jj * BK * 4;
-        const uint32_t vo = avoff[i];
-        asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(vo), "s"(sb),
-                     "s"(base + i * T * 16) : "memory", "m0");
+        ta_load_lds16(abase0 + (uint64_t)jj * BK * 4, avoff[i], base + i * T * 16);
       } else {
-        const char *sb = bbase0 + (uint64_t)jj * b_stage;
-        const uint32_t vo = bvoff[i - A_LD];
-        asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(vo),
-                     "s"(sb), "s"(base + A_BYTES + (i - A_LD) * T * 16) : "memory", "m0");
+        ta_load_lds16(bbase0 + (uint64_t)jj * b_stage, bvoff[i - A_LD], base + A_BYTES + (i - A_LD) * T * 16);
       }
     };
     // i-th LDS read of stage `stg` (compile time) into register set `set`.

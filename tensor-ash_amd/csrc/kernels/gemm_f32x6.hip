@@ -83,9 +83,7 @@ template <int BM, int BN, int WGM, int WGN, int G, int NS, bool TWO> struct Gemm
 #pragma unroll
       for (int i = 0; i < LD; ++i) {
         const uint32_t l = lds0 + st * STAGE + (i * W + wave) * 1024u;
-        const char *s = src[i];
-        asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lo), "s"(s), "s"(l)
-                     : "memory", "m0");
+        ta_load_lds16(src[i], lo, l);
         src[i] += G * STEP;
       }
     };
