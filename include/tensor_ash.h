@@ -552,7 +552,8 @@ int ta_q8_cache_write(const ta_executor *exec, const ta_tensor *k, const ta_tens
 
 /* Reads positions first .. first + positions - 1 back, to the same positions
  * of the dense caches kt [kv_heads, head_dim, T] and v [kv_heads, T,
- * head_dim] (f32, exactly; or f16, RNE; alike), which keep what they hold
+ * head_dim] (f32, exactly; or f16, RNE, but 65532, for which f16's largest
+ * magnitudes may stand, as 65504; alike), which keep what they hold
  * elsewhere. */
 typedef struct ta_q8_read_desc {
   uint32_t first;

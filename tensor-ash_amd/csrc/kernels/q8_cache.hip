@@ -165,6 +165,15 @@ template <int DH, bool F16> TA_DEVICE void q8_write(const Q8WriteArgs &p) {
 TA_DEVICE float code_value(uint32_t word, int byte, float s) { return (float)(int8_t)(word >> (8 * byte)) * s; }
 TA_DEVICE float scale_value(uint32_t half) { return __uint_as_float(half << 16); }
 
+// Rows whose largest magnitude is one of f16's top eight have the scale 516,
+// and the code 127 then stands for 65532, which f16 would round to infinity:
+// as f16 it is f16's largest, 65504.  (No other scale and code give 65532.)
+constexpr float kF16TopScale = 516.0f, kF16Top = 65504.0f;
+TA_DEVICE bool f16_top(const float (&s)[4]) {
+  return s[0] == kF16TopScale || s[1] == kF16TopScale || s[2] == kF16TopScale || s[3] == kF16TopScale;
+}
+TA_DEVICE float f16_within(float v) { return fabsf(v) == 127.0f * kF16TopScale ? copysignf(kF16Top, v) : v; }
+
 // 128 positions (four blocks) of a kv head.
 template <int DH, bool F16> TA_DEVICE void q8_read(const Q8ReadArgs &p) {
   __shared__ __attribute__((aligned(16))) uint8_t turn[4 * DH * kRow];
@@ -200,7 +209,7 @@ template <int DH, bool F16> TA_DEVICE void q8_read(const Q8ReadArgs &p) {
     const u32x2 raw = *reinterpret_cast<const u32x2 *>(rec + 64u * DH + ta_q8_slot(4u * a) * 2u);
     const float s[4] = {scale_value(raw[0] & 0xFFFFu), scale_value(raw[0] >> 16), scale_value(raw[1] & 0xFFFFu),
                         scale_value(raw[1] >> 16)};
-    const bool all = pos >= p.first && pos + 4u <= end;
+    const bool all = pos >= p.first && pos + 4u <= end, top = F16 && f16_top(s);
     const uint64_t row0 = ((uint64_t)head * DH + part * 16u) * p.t_dst + pos;
 #pragma unroll
     for (int d = 0; d < 16; ++d) {
@@ -208,6 +217,11 @@ template <int DH, bool F16> TA_DEVICE void q8_read(const Q8ReadArgs &p) {
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         v[r] = code_value(c[r][d / 4], d & 3, s[r]);
+      if (top) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          v[r] = f16_within(v[r]);
+      }
       const uint64_t at = row0 + (uint64_t)d * p.t_dst;
       if (all) {
         if constexpr (F16)
@@ -244,6 +258,7 @@ template <int DH, bool F16> TA_DEVICE void q8_read(const Q8ReadArgs &p) {
                                                        slot * 2u);
     const float s[4] = {scale_value(raw[0] & 0xFFFFu), scale_value(raw[0] >> 16), scale_value(raw[1] & 0xFFFFu),
                         scale_value(raw[1] >> 16)};
+    const bool top = F16 && f16_top(s);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       if (pos + r < p.first || pos + r >= end)
@@ -254,6 +269,13 @@ template <int DH, bool F16> TA_DEVICE void q8_read(const Q8ReadArgs &p) {
       for (int d = 0; d < 4; ++d) {
         lo[d] = code_value(c[d], r, s[r]);
         hi[d] = code_value(c[4 + d], r, s[r]);
+      }
+      if (top) {
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          lo[d] = f16_within(lo[d]);
+          hi[d] = f16_within(hi[d]);
+        }
       }
       if constexpr (F16) {
         const f16x4 l = __builtin_convertvector(lo, f16x4), u = __builtin_convertvector(hi, f16x4);

@@ -186,6 +186,33 @@ def test_q8_write_at_a_cell(ta, ex):
         assert same(read_back(ta, ex, cache, False, t_max)[1], want, False), at
 
 
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("dh,first", [(64, 0), (128, 3)])
+def test_q8_rows_that_f16_holds_read_back_finite(ta, ex, f16, dh, first):
+    """The scale of a row whose largest magnitude is among f16's top eight is
+    516, and 127 times that is past f16's largest: it reads back as that one.
+    Rows past f16 read back as infinities still, rows with a NaN as NaN."""
+    tops = np.arange(65280, 65505, 32, dtype=np.float32)
+    n = 2 * tops.size + 3
+    x = np.random.default_rng(dh).standard_normal((n, dh)).astype(np.float32)
+    x[:tops.size, 7], x[tops.size:2 * tops.size, dh - 1] = tops, -tops
+    x[-1, 5] = np.nan
+    if f16:
+        x = x.astype(np.float16).astype(np.float32)
+    else:
+        x[-2, 9], x[-3, 9] = 7e4, -1e9
+    want = stands_for(x)
+    assert (np.abs(want[:2 * tops.size]).max(-1) == 65532).all()
+    cache = ex.q8_cache(1, dh, n)
+    t = ex.tensor_from(x, f16=f16)
+    ex.q8_cache_write(t, t, cache, ta.Q8WriteDesc(n))
+    k, v = read_back(ta, ex, cache, True, n - first, first)
+    want = np.where(np.abs(want) == 65532, np.sign(want) * 65504, want)[first:]
+    with np.errstate(over="ignore"):
+        assert same(k[0, :, first:].T, want, True) and same(v[0, first:], want, True)
+    assert np.isfinite(v[0, first:2 * tops.size]).all() and np.isinf(v[0]).any() == (not f16)
+
+
 # ------------------------------------------------------------------- RoPE
 
 
