@@ -1278,14 +1278,16 @@ template <int DH, int KP> struct TreeF32 {
     for (int s = 0; s < HALF; ++s)
       r[s] = base[(uint32_t)s * p.t_max + lane];
   }
-  static TA_DEVICE void load_v(const float *v, const TreeArgs &p, const Place &w, uint32_t k0, vrow (&r)[16]) {
+  // Memory past the drafts may hold anything (0 * inf is not 0): for its keys,
+  // whose weights are zeros, the last draft's row.
+  static TA_DEVICE void load_v(const float *v, const Place &w, uint32_t k0, vrow (&r)[16]) {
     const float *base = v + (uint64_t)k0 * DH;
-    const bool whole = k0 + BK <= p.t_max;
+    const bool whole = k0 + BK <= w.total;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       uint32_t key = 8u * (e / 4) + 4u * w.h + e % 4;
       if (!whole)
-        key = min(key, p.t_max - 1u - k0);
+        key = min(key, w.total - 1u - k0);
       r[e] = *reinterpret_cast<const vrow *>(base + key * DH + w.j * DB);
     }
   }
@@ -1305,7 +1307,7 @@ template <int DH, int KP> struct TreeF32 {
     uint32_t b = b0 + wave;
     if (b < b1) {
       load_k(kt, p, w, b * BK, rk);
-      load_v(vv, p, w, b * BK, rv);
+      load_v(vv, w, b * BK, rv);
     }
     // value d = s + h dh / 2 of row r: [s / 4][lane][s % 4]
     load_q<DH, false>(p, w, [&](uint32_t part, uint32_t r, const float(&x)[DH / 8]) __attribute__((always_inline)) {
@@ -1348,7 +1350,7 @@ template <int DH, int KP> struct TreeF32 {
           st.o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(rv[e][d], x, st.o[d], 0, 0, 0);
       }
       if (b + KP < b1)
-        load_v(vv, p, w, (b + KP) * BK, rv);
+        load_v(vv, w, (b + KP) * BK, rv);
     }
     if (__any(w.live && !st.finite()))
       whole_values<DH, kF32, false>(p, w, st, (b0 + wave) * BK, b1 * BK, KP * BK, BK);

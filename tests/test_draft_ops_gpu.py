@@ -717,6 +717,21 @@ def test_tree_attention_f16_weights_in_two_pieces(ta, ex, dh, group, tokens, t_m
     assert (np.abs(got - out) <= tol).all(), float((np.abs(got - out) / tol).max())
 
 
+@pytest.mark.parametrize("cache,f16", KINDS)
+@pytest.mark.parametrize("dh,group,tokens,n0,extra", [(64, 2, 6, 100, 40), (128, 4, 3, 300, 2), (128, 8, 16, 240, 1)])
+def test_tree_attention_bits_without_what_lies_behind(ta, ex, cache, f16, dh, group, tokens, n0, extra):
+    """Memory behind the drafts may hold anything: not a bit of the result,
+    nor the way it is taken, depends on it."""
+    got = []
+    for bad in (0.0, 1.0, np.inf, np.nan):
+        c = Case(ta, ex, cache, f16, dh, 2, group, tokens, n0, extra)
+        c.k[c.n:] = c.v[c.n:] = bad
+        got.append(c.put().run())
+    c.check(got[0])
+    for g in got[1:]:
+        assert np.array_equal(got[0], g)
+
+
 # ------------------------------------------------------------- used together
 
 
