@@ -91,6 +91,16 @@ TA_DEVICE void in_order() { __builtin_amdgcn_sched_barrier(0); }
 // block takes four times its registers).
 template <class T> TA_DEVICE void from_here(T &x) { asm volatile("" : "+v"(x)); }
 
+// scale * log2 e as a positive number, its sign for q.  A scale of zero becomes
+// zeros of q, so that every finite score is 0 and a masked one stays -inf.
+// Below f32's smallest normal the product is off by 2^-150, so an exponent by
+// 2^-22 at most, where q . k is near f32's largest.
+TA_DEVICE float split_scale(float scale, float &sign) {
+  const float s2 = scale * 1.44269504088896340736f;
+  sign = s2 < 0.0f ? -1.0f : s2 > 0.0f ? 1.0f : 0.0f;
+  return s2 != 0.0f ? s2 * sign : kMinScale;
+}
+
 TA_DEVICE float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 // Maximum / sum over the two lanes (halves of the wave) of a row.
 TA_DEVICE float other_half(float x) {
@@ -574,8 +584,8 @@ template <int DH, bool IO16, int KP> struct TreeQ8 {
     const Place w(p, 1, 0);
     uint32_t b0, b1;
     chunk_blocks(p, w, TA_Q8_BLOCK, b0, b1);
-    const float s2 = p.scale * 1.44269504088896340736f, sign = s2 < 0.0f ? -1.0f : 1.0f;
-    const float scale2 = fmaxf(s2 * sign, kMinScale);
+    float sign;
+    const float scale2 = split_scale(p.scale, sign);
     // The first block before q, and the mask (in host memory) after both: a
     // load is waited for with all before it.
     const uint8_t *base = p.cache + (uint64_t)w.kvh * p.blocks * ta_q8_record(DH);
@@ -795,8 +805,8 @@ template <int DH, bool IO16, int KP> struct TreeQ8Few {
       load_k(rec(b), lane, r);
       load_v(rec(b), lane, r);
     }
-    const float s2 = p.scale * 1.44269504088896340736f, sign = s2 < 0.0f ? -1.0f : 1.0f;
-    const float scale2 = fmaxf(s2 * sign, kMinScale);
+    float sign;
+    const float scale2 = split_scale(p.scale, sign);
     u32x4 *qs = reinterpret_cast<u32x4 *>(smem);
     // q's operands: 8 values from d = 8 i on of row r are step 2 (i / 8) + i %
     // 2 of lane 16 (i / 2 % 4) + r
@@ -1298,8 +1308,8 @@ template <int DH, int KP> struct TreeF32 {
     const Place w(p, 1, 0);
     uint32_t b0, b1;
     chunk_blocks(p, w, BK, b0, b1);
-    const float s2 = p.scale * 1.44269504088896340736f, sign = s2 < 0.0f ? -1.0f : 1.0f;
-    const float scale2 = fmaxf(s2 * sign, kMinScale);
+    float sign;
+    const float scale2 = split_scale(p.scale, sign);
     const float *kt = static_cast<const float *>(p.kt) + (uint64_t)w.kvh * DH * p.t_max;
     const float *vv = static_cast<const float *>(p.v) + (uint64_t)w.kvh * p.t_max * DH;
     float rk[HALF];

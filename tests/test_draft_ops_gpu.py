@@ -732,6 +732,25 @@ def test_tree_attention_bits_without_what_lies_behind(ta, ex, cache, f16, dh, gr
         assert np.array_equal(got[0], g)
 
 
+@pytest.mark.parametrize("cache,f16", [("f32", False), ("q8", False), ("q8", True)])
+@pytest.mark.parametrize("group", [2, 20])
+@pytest.mark.parametrize("scale", [0.0, 1e-45, 1e-40, -1e-38])
+def test_tree_attention_small_scales_of_large_scores(ta, ex, cache, f16, group, scale):
+    """A scale of zero, or below f32's smallest normal, over q . k near f32's
+    largest: what the formula has.  (scale log2 e then has an error of its own
+    of 2^-150; times |q . k| < 2^123 that is below the exponential's 4 u.)"""
+    c = Case(ta, ex, cache, f16, 64, 2, group, 5, 120)
+    if not f16:
+        c.q *= 1e15
+    c.k *= np.float32(1e36 if f16 else 1e21)
+    c.put()
+    c.scale = float(np.float32(scale))
+    q = c.q.astype(np.float64).reshape(5, 2, group, 64)
+    top = np.abs(np.einsum("tgad,ngd->tgan", q, c.values()[0])).max()
+    assert 2.0 ** 118 < top < 2.0 ** 126
+    c.check(c.run())
+
+
 # ------------------------------------------------------------- used together
 
 
