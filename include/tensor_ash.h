@@ -581,7 +581,7 @@ int ta_q8_cache_read(const ta_executor *exec, const ta_q8_cache *cache, const ta
 typedef struct ta_tree_desc {
   uint32_t kv_len;
   uint32_t tokens;
-  float scale;       /* 1/sqrt(dh) for standard attention */
+  float scale;       /* 1/sqrt(dh) for standard attention; scale * log2(e) within f32 */
   uint32_t reserved; /* must be zero */
   uint64_t q_offset, q_stride;
   uint64_t pos_addr;

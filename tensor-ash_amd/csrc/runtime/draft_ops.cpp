@@ -170,6 +170,8 @@ TreePlan tree_plan(const std::string &op, uint32_t cus, TreeCache kind, const Ca
     fail(op + ": kv_len " + str(d.kv_len) + " + tokens " + str(d.tokens) + " exceeds T_max " + str(c.t_max));
   if (!std::isfinite(d.scale))
     fail(op + ": scale must be finite");
+  if (!std::isfinite(d.scale * 1.44269504088896340736f)) // the kernels' exponents are in base 2
+    fail(op + ": scale " + std::to_string(d.scale) + " times log2(e) is past f32");
   const uint64_t per_head = (uint64_t)d.tokens * c.kv_heads * c.dh;
   if (out.len() == 0 || out.len() % per_head != 0)
     fail(op + ": out " + fmt_shape(out.shape) + " must hold tokens*H*dh elements (tokens " + str(d.tokens) + ", dh " +

@@ -204,6 +204,20 @@ static void test_tree() {
               }
 }
 
+static void test_tree_scale_range() {
+  const Operand x = f32({1, 64});
+  TreeDesc d;
+  d.tokens = 1;
+  auto error = [&](float scale) {
+    d.scale = scale;
+    return error_of([&] { tree_plan("op", 256, TreeCache::F32, {1, 64, 1}, x, x, std::nullopt, d); });
+  };
+  for (float s : {0.0f, 1e-45f, 1.0f, 2.3e38f, -2.3e38f})
+    CHECK(error(s).empty());
+  for (float s : {2.4e38f, -2.4e38f, 3.4e38f})
+    CHECK(has(error(s), "times log2(e) is past f32"));
+}
+
 static void test_rope_axes() {
   RopeAxesDesc d;
   d.heads = 4;
@@ -252,6 +266,7 @@ static void test_rope_axes() {
 int main() {
   test_q8();
   test_tree();
+  test_tree_scale_range();
   test_rope_axes();
   std::printf("%d checks, %d failed%s\n", g_pass + g_fail, g_fail, g_fail ? "" : ": all passed");
   return g_fail ? 1 : 0;
