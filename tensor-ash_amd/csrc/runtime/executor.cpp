@@ -1631,12 +1631,14 @@ struct ExecutorImpl {
   }
   void record_elem(const ElemLaunches &ls, const Scratch &scratch, hipStream_t stream) const {
     for (const ElemLaunch &l : ls) {
-      std::vector<uint8_t> args = l.args;
-      if (l.partial_bytes) {
-        if (scratch.partial_bytes < l.partial_bytes)
-          fail("internal: scratch of " + l.symbol + " not reserved");
-        std::memcpy(args.data() + l.partial_at, &scratch.partial, sizeof(void *));
+      if (!l.partial_bytes) {
+        launch(l.symbol, l.groups, l.gy, 1, l.threads, const_cast<uint8_t *>(l.args.data()), stream);
+        continue;
       }
+      if (scratch.partial_bytes < l.partial_bytes)
+        fail("internal: scratch of " + l.symbol + " not reserved");
+      std::vector<uint8_t> args = l.args;
+      std::memcpy(args.data() + l.partial_at, &scratch.partial, sizeof(void *));
       launch(l.symbol, l.groups, l.gy, 1, l.threads, args.data(), stream);
     }
   }
