@@ -488,7 +488,8 @@ typedef struct Q8ReadArgs {
 // kv head), in that order from the slowest; the join's are (row tile, 32 head
 // dimensions, kv head).
 // With several chunks a workgroup leaves {o, m, l} of its rows in `partial`
-// (ta_tree_combine), else it writes out.  q element (t, head, d) sits at
+// (ta_tree_combine), else it writes out; row_tiles, of a kv head, sizes that and
+// the join's grid.  q element (t, head, d) sits at
 // q_offset + t * q_stride + head * dh + d; out is dense.
 #define TA_TREE_MAX_TOKENS 64u
 #define TA_TREE_MAX_CHUNKS 64u

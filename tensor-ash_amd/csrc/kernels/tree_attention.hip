@@ -209,61 +209,52 @@ template <int DH, int KIND> TA_DEVICE uint32_t out_dim(int b, int q, int r, uint
 // The states of the KP waves of a row tile become one; with one chunk the
 // result goes to `out`, else {o, m, l} to the row tile's scratch.  Wave `part`
 // of the KP sums every KP-th register quad.
-template <int DH, int KP> constexpr int merge_floats() { return KP == 1 ? 0 : KP * (DH / 2) * 64 + 2 * KP * 64; }
+template <int DH, int KP> constexpr int merge_floats() { return KP * (DH / 2) * 64 + 2 * KP * 64; }
 
 template <int DH, int KIND, bool IO16, int KP>
 TA_DEVICE void finish(const TreeArgs &p, const Place &w, State<DH> &st, uint32_t part, float *smem) {
   constexpr int DB = DH / 32, QUADS = DB * 4, OWN = KP < 4 ? 4 / KP : 1; // quads q = part + KP i < 4
-  static_assert(KP == 1 || KP == 2 || KP == 4 || KP == 8, "quads split evenly");
-  float top = st.m, l = st.l + other_half(st.l);
-  f32x4 v[OWN][DB];
-  if constexpr (KP == 1) {
+  static_assert(KP == 2 || KP == 4 || KP == 8, "quads split evenly");
+  float l = st.l + other_half(st.l);
+  f32x4 *mo = reinterpret_cast<f32x4 *>(smem);
+  float *mm = smem + KP * (DH / 2) * 64, *ml = mm + KP * 64;
+  __syncthreads(); // the operands in this memory are done with
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
 #pragma unroll
     for (int q = 0; q < 4; ++q)
+      mo[(part * QUADS + b * 4 + q) * 64u + w.lane] =
+          f32x4{st.o[b][4 * q], st.o[b][4 * q + 1], st.o[b][4 * q + 2], st.o[b][4 * q + 3]};
+  mm[part * 64u + w.lane] = st.m;
+  ml[part * 64u + w.lane] = l;
+  __syncthreads();
+  float a[KP], top = mm[w.lane];
 #pragma unroll
-      for (int b = 0; b < DB; ++b)
-        v[q][b] = f32x4{st.o[b][4 * q], st.o[b][4 * q + 1], st.o[b][4 * q + 2], st.o[b][4 * q + 3]};
-  } else {
-    f32x4 *mo = reinterpret_cast<f32x4 *>(smem);
-    float *mm = smem + KP * (DH / 2) * 64, *ml = mm + KP * 64;
-    __syncthreads(); // the operands in this memory are done with
+  for (uint32_t i = 1; i < KP; ++i)
+    top = fmaxf(top, mm[i * 64u + w.lane]);
+  l = 0.0f;
 #pragma unroll
-    for (int b = 0; b < DB; ++b)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        mo[(part * QUADS + b * 4 + q) * 64u + w.lane] =
-            f32x4{st.o[b][4 * q], st.o[b][4 * q + 1], st.o[b][4 * q + 2], st.o[b][4 * q + 3]};
-    mm[part * 64u + w.lane] = st.m;
-    ml[part * 64u + w.lane] = l;
-    __syncthreads();
-    float a[KP];
-    top = mm[w.lane];
-#pragma unroll
-    for (uint32_t i = 1; i < KP; ++i)
-      top = fmaxf(top, mm[i * 64u + w.lane]);
-    l = 0.0f;
-#pragma unroll
-    for (uint32_t i = 0; i < KP; ++i) {
-      a[i] = exp2_fast(mm[i * 64u + w.lane] - top);
-      l = fmaf(ml[i * 64u + w.lane], a[i], l);
-    }
-    if (KP > 4 && part >= 4u)
-      return;
-#pragma unroll
-    for (int o = 0; o < OWN; ++o)
-#pragma unroll
-      for (int b = 0; b < DB; ++b) {
-        const uint32_t at = b * 4u + part + KP * o;
-        v[o][b] = mo[at * 64u + w.lane] * a[0];
-#pragma unroll
-        for (uint32_t i = 1; i < KP; ++i) {
-          const f32x4 x = mo[(i * QUADS + at) * 64u + w.lane];
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            v[o][b][r] = fmaf(x[r], a[i], v[o][b][r]);
-        }
-      }
+  for (uint32_t i = 0; i < KP; ++i) {
+    a[i] = exp2_fast(mm[i * 64u + w.lane] - top);
+    l = fmaf(ml[i * 64u + w.lane], a[i], l);
   }
+  if (KP > 4 && part >= 4u)
+    return;
+  f32x4 v[OWN][DB];
+#pragma unroll
+  for (int o = 0; o < OWN; ++o)
+#pragma unroll
+    for (int b = 0; b < DB; ++b) {
+      const uint32_t at = b * 4u + part + KP * o;
+      v[o][b] = mo[at * 64u + w.lane] * a[0];
+#pragma unroll
+      for (uint32_t i = 1; i < KP; ++i) {
+        const f32x4 x = mo[(i * QUADS + at) * 64u + w.lane];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          v[o][b][r] = fmaf(x[r], a[i], v[o][b][r]);
+      }
+    }
   if (!w.live)
     return;
   if (p.chunks > 1) {

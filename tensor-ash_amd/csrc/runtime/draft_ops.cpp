@@ -222,8 +222,8 @@ TreePlan tree_plan(const std::string &op, uint32_t cus, TreeCache kind, const Ca
   p.stage.threads = shape.threads;
   if (a.chunks > 1) {
     p.combine.symbol = "ta_tree_combine_" + name;
-    p.combine.gx = (uint32_t)(tiles * (c.dh / 32) * c.kv_heads);
-    p.partial_bytes = tiles * a.chunks * c.kv_heads * ta_tree_partial(c.dh) * 4;
+    p.combine.gx = a.row_tiles * (c.dh / 32) * c.kv_heads;
+    p.partial_bytes = (uint64_t)a.row_tiles * a.chunks * c.kv_heads * ta_tree_partial(c.dh) * 4;
   }
   return p;
 }
