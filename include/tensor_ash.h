@@ -575,8 +575,10 @@ int ta_q8_cache_read(const ta_executor *exec, const ta_q8_cache *cache, const ta
  * [tokens, H * dh] (any shape of that length, and its H a multiple of
  * H_kv), f32, or f16 over an f16 or 8-bit cache; q has out's type, its
  * element (t, head, d) at q_offset + t * q_stride + head * dh + d (q_stride
- * 0: H * dh), so it may be part of a fused QKV product.  dh 64 or 128; over
- * an 8-bit cache |q| * 127 * dh has to stay within f32. */
+ * 0: H * dh), so it may be part of a fused QKV product.  dh 64 or 128.  q . k
+ * and 16 times the sum of |v| over the positions seen have to stay within
+ * f32, over an 8-bit cache |q| * 127 * dh too; what does not comes out as
+ * infinities or NaN. */
 #define TA_TREE_MAX_TOKENS 64u
 typedef struct ta_tree_desc {
   uint32_t kv_len;

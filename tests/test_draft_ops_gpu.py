@@ -751,6 +751,22 @@ def test_tree_attention_small_scales_of_large_scores(ta, ex, cache, f16, group, 
     c.check(c.run())
 
 
+@pytest.mark.parametrize("group", [2, 20])
+def test_tree_attention_q8_largest_q(ta, ex, group):
+    """|q| * 127 * dh close under f32's largest, against a row of K whose codes
+    are all 127, and V whose sum with weights of 16 is close under it too."""
+    c = Case(ta, ex, "q8", False, 64, 2, group, 5, 120)
+    c.q *= np.float32(4.1e34) / np.abs(c.q).max()
+    c.q[0] = 4.1e34
+    c.k *= np.float32(1e-29)
+    c.k[3] = 127.0 * 2.0 ** -100
+    c.v *= np.float32(3.3e38 / 16) / np.abs(c.v).sum(0).max()
+    c.put()
+    c.scale = float(np.float32(1e-7))
+    assert (c.values()[0][3] == 127.0 * 2.0 ** -100).all()
+    c.check(c.run())
+
+
 # ------------------------------------------------------------- used together
 
 
