@@ -9,16 +9,16 @@
 // s having 8 bits, s * 127 (15 bits) and s * (c + 1/2) (16 bits) are exact
 // in f32, so both decisions are made exactly: s from the f32 quotient cut to
 // 8 bits and one comparison, c from the f32 quotient (q8_code).  s * c is exact
-// in f32 as well.  A row that holds an infinity or a NaN gets a NaN scale: all of it reads back
-// as NaN.  Half a step is at most 1/254 * (1 + 2^-7) of the row's largest
-// value.
+// in f32 as well.  A row that holds an infinity or a NaN gets a NaN scale: all
+// of it reads back as NaN.  Half a step is at most 1/254 * (1 + 2^-7) of the
+// row's largest value.
 //
 // Both kernels are bound by HBM on long runs of positions (16384 of 8 heads of
-// 128, f16: written in 17.7 us, 101 MB at 5.7 TB/s, the vector units busy in 88%
-// of it; read back in 16.2 us, the codes still in the caches) and by their
-// launch on short ones (one token: 2.6 us).  A workgroup writes one block of 32 positions of one head, so that
-// its bytes are its own: V's codes lie across positions, and no two
-// workgroups write one 16-byte piece.
+// 128, f16: written in 17.9 us, 101 MB at 5.6 TB/s, the vector units busy in 90%
+// of it; read back in 16.6 us, the codes still in the caches) and by their
+// launch on short ones (one token: 3.0 us).  A workgroup writes one block of 32
+// positions of one head, so that its bytes are its own: V's codes lie across
+// positions, and no two workgroups write one 16-byte piece.
 #include "common.h"
 
 namespace {

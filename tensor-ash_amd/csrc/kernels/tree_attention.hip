@@ -14,7 +14,8 @@
 // Work split.  The rows of a kv head, (token, head of its group), are taken
 // 32 at a time, an MFMA's columns (16 for at most 16 rows of the 8-bit cache).
 // A workgroup is one, two or four such row tiles over one chunk of the
-// positions, about one workgroup to a CU.  The waves of a row tile share the
+// positions (64 chunks at most), no more workgroups than CUs where the row
+// tiles alone are fewer.  The waves of a row tile share the
 // chunk's keys, each with its own m, l and output, and meet in LDS at the end.
 // With several chunks, workgroups leave their rows' {o, m, l} in scratch and
 // ta_tree_combine joins them in chunk order.  No atomics: results do not
@@ -45,19 +46,19 @@
 // (0 * inf), and where a mask hides it nothing may come of it: a wave whose
 // rows come out non-finite takes its keys again, whole values on the vector
 // units, masked ones skipped (64 drafts, 32704 positions, 32 / 8 heads, dh
-// 128, f16, an infinity in every head: 1.7 ms; 0.05 without).
+// 128, f16, an infinity in every head: 1.7 ms; 0.07 without).
 //
 // Bound and measured (kernel and join, us; copy 5.1 TB/s, f16 matrix product
 // 1030 TFLOP/s):
-//   f16, 64 drafts, 32704 positions, 32 / 8 heads, dh 128: 47.6 + 4.9, 720
-//     TFLOP/s and 2.8 TB/s; matrix cores (38% busy) and vector units (39%), one
-//     after the other within a wave;
-//   8-bit, 1 token, 32767 positions, 32 / 8 heads, dh 128, f32: 15.3 + 5.3,
+//   f16, 64 drafts, 32704 positions, 32 / 8 heads, dh 128: 60.3 + 4.8, 570
+//     TFLOP/s and 2.2 TB/s (47.6 with weights in one piece, 2^-11 off); matrix
+//     cores (46% busy) and vector units (43%), one after the other in a wave;
+//   8-bit, 1 token, 32767 positions, 32 / 8 heads, dh 128, f32: 15.6 + 5.4,
 //     4.4 TB/s; HBM;
-//   8-bit, 26 drafts, 8191 positions, 32 / 4 heads, dh 64, f16: 11.0 + 4.0;
+//   8-bit, 26 drafts, 8191 positions, 32 / 4 heads, dh 64, f16: 11.8 + 4.0;
 //     exponentials and conversions (4.6 MB);
 //   f16 cache of odd length, f32, 25 drafts, 4999 positions, 32 / 8 heads, dh
-//     128: 19.0 + 4.1; five tiles to a chunk, latency of start, tiles and end;
+//     128: 19.5 + 4.1; five tiles to a chunk, latency of start, tiles and end;
 //   f32, 8 drafts, 1016 positions, 32 / 4 heads, dh 64: 7.0 + 4.0; latency.
 #include "common.h"
 
@@ -929,14 +930,13 @@ template <int DH, bool IO16, bool DIRECT, int QB, int KP, int BKW> struct TreeF1
   // The waves of the second key part run their output product one tile late (a
   // third buffer keeps its V).  That keeps the two waves of a SIMD in different
   // phases, which on its own was no gain (64 drafts, 32704 positions, 32 / 8
-  // heads, f16: 58 us against 55), but where K goes through registers beside
+  // heads, f16, weights in one piece: 58 us against 55), but where K goes through registers beside
   // f32 q's three pieces the later use of V's operands is what keeps the loop
   // within its registers (64 drafts, 16000 positions: 61 us, 93 without).
   static constexpr bool LATE = T == 512 && !DIRECT && !IO16 && DH == 128;
   // Tiles in flight.  Two hide more of HBM's latency where a CU holds one
-  // workgroup anyway (64 drafts, 32704 positions, 32 / 8 heads, dh 128, f16: 70
-  // us behind other work, 76 with one, 71 with three; 55 all three when called
-  // again).  Four waves lose by them (16 drafts, 32000 positions, dh 64: 26.4
+  // workgroup anyway (64 drafts, 32704 positions, 32 / 8 heads, dh 128, f16: 72
+  // us behind other work, 76 with one; 69 and 68 when called again).  Four waves lose by them (16 drafts, 32000 positions, dh 64: 26.4
   // us, 23.5 with one).
   static constexpr int FLIGHT = DIRECT && T == 512 ? 2 : 1;
   static constexpr int BUFS = LATE || FLIGHT == 2 ? 3 : 2;

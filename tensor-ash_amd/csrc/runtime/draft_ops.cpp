@@ -136,10 +136,13 @@ struct TreeShape {
 //    16 rows or fewer: 16.3 / 16.9, on a 32-row tile 18.1 / 19.4.
 //  * f16 cache, rows x positions below 2^20: few positions to a chunk, so that
 //    the larger workgroups' start weighs more than what they share (128 rows
-//    of dh 128 at 4000 positions: two tiles 16.9 / 20.7, four 20.4 / 25.0; of
-//    dh 64, one tile 13.9 / 15.6, four 14.9 / 17.6).  Beyond, four tiles at
-//    once: 128 rows of dh 128 at 65000 80.3 / 106.0 -> 56.7 / 92.6, 256 rows of
-//    dh 64 at 8000 23.2 / 27.8 -> 18.8 / 25.2.
+//    of dh 128 at 4000 positions: two tiles 17.3 / 20.7, four 21.9 / 25.6; of
+//    dh 64, one tile 14.0 / 15.8, four 16.7 / 18.6).  Beyond, four tiles at
+//    once: 128 rows of dh 128 at 65000 100.5 / 104.1 -> 75.5 / 92.8, 256 rows of
+//    it at 32768 77.5 / 101.7 -> 65.1 / 88.8, 256 rows of dh 64 at 8000 22.6 /
+//    26.4 -> 20.6 / 24.2.  At the border itself dh 64 is level (16.4 / 19.2,
+//    16.6 / 19.0) and two tiles of dh 128 are still ahead (20.8 / 26.2, four
+//    23.3 / 27.7 at 128 rows and 8192).
 //  * f16 cache, two tiles to a workgroup: dh 128 only (64 rows at 16000:
 //    22.8 / 28.3, one tile 25.0 / 32.2; dh 64 18.3 / 20.5, one tile 16.9 / 19.3).
 TreeShape tree_shape(TreeCache kind, const CacheShape &c, uint64_t rows, uint64_t tiles, uint64_t keys) {
@@ -194,8 +197,10 @@ TreePlan tree_plan(const std::string &op, uint32_t cus, TreeCache kind, const Ca
   const TreeShape shape = tree_shape(kind, c, d.tokens * group, tiles, keys);
   const uint64_t groups = ceil_div(tiles, shape.tiles);
   // Chunks: at most a workgroup for every CU (280 for 256 took 16.4 us where
-  // 252 took 11.5), each with shape.keys keys at least.  More
-  // cost more than they hide (us at 24 / 32 / 48 / 64 chunks, 8 kv heads of dh
+  // 252 took 11.5), each with shape.keys keys at least where the length is
+  // known.  With a cell it is the capacity's: 500 positions in a cache of 32768
+  // (8 kv heads of 4, dh 128) take 15.5 us for 10.3 by number with one token
+  // over 8 bits, 18.8 for 15.0 with 64 over f16.  More chunks cost more than they hide (us at 24 / 32 / 48 / 64 chunks, 8 kv heads of dh
   // 128, 32000 positions: f16, 32 rows 30.4 / 30.2 / 37.7 / 36.2, 64 rows 33.9 /
   // 30.8 / 33.8 / 35.3; f32 q on f16, 128 rows 63.8 / 57.2 / 75.1 / 69.8; 8-bit,
   // 32 rows 31.7 / 28.0 / 31.0 / 29.4), and so do chunks of less (f16, 64 rows,
